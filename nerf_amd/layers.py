@@ -15,6 +15,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
@@ -25,6 +26,7 @@ ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 
 
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+_transforms = torch._C._functorch.peek_interpreter_stack
 
 
 def _launch(device, fn, what, *args):
@@ -75,6 +77,14 @@ def _at(t):
     return None if t is None else t.data_ptr()
 
 
+def _recorded(a, b, c=None):
+    """Whether a call goes through its autograd function: where a gradient will be asked for, and inside forward-mode differentiation
+    (whose tangents travel beside tensors that need no gradient) and torch.func's transforms.  The kernels write through raw pointers,
+    which neither of those sees: the function refuses them by name, as it has no `jvp` and no `setup_context`."""
+    return (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad or (c is not None and c.requires_grad))
+            or forward_ad._current_level >= 0 or _transforms() is not None)
+
+
 def _first_order(fn):
     """Backward passes are kernels, not differentiable again: `once_differentiable`, which says so where a graph of the backward pass
     is being made, and which the ordinary backward pass need not go through (it takes 5 us of a small layer's 50)."""
@@ -92,18 +102,17 @@ def embedding(index, table, scale=1.0):
 
     An index outside [0, n_entries) gives a row of zeros and no gradient (nets.py:132 raises there; a kernel cannot).  The
     table's gradient is dense and adds the rows of each entry in ascending order of their place in `index`."""
+    call = _EmbeddingFn.apply if _recorded(table, index) else _embedding_fwd
+    return call(table, index, float(scale))
+
+
+def _embedding_fwd(table, index, scale):
     if index.dtype != torch.int64:
         raise TypeError('index must be int64 (got %s)' % index.dtype)
     if table.dim() != 2 or table.shape[1] < 1:
         raise ValueError('table must be [n_entries, dim] (got %s)' % (tuple(table.shape),))
     _dtype(table, 'table')
     device = _device('embedding', index, table)
-    if table.requires_grad and torch.is_grad_enabled():
-        return _EmbeddingFn.apply(table, index, float(scale), device)
-    return _embedding_fwd(table, index, float(scale), device)
-
-
-def _embedding_fwd(table, index, scale, device):
     table, index = table.contiguous(), index.contiguous()
     entries, dim = table.shape
     out = table.new_empty(index.shape + (dim,))
@@ -114,10 +123,10 @@ def _embedding_fwd(table, index, scale, device):
 
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, index, scale, device):
+    def forward(ctx, table, index, scale):
         ctx.save_for_backward(index)
-        ctx.shape, ctx.scale, ctx.device = table.shape, scale, device
-        return _embedding_fwd(table, index, scale, device)
+        ctx.shape, ctx.scale = table.shape, scale
+        return _embedding_fwd(table, index, scale)
 
     @_first_order
     def backward(ctx, dout):
@@ -128,9 +137,9 @@ class _EmbeddingFn(torch.autograd.Function):
         dtable = d.new_empty((entries, dim))
         n = lib().nerf_embedding_bwd_workspace_bytes(code, entries, dim, rows)
         ws = _workspace(n, 'nerf_embedding_bwd', d)
-        _launch(ctx.device, lib().nerf_embedding_bwd, 'nerf_embedding_bwd', index.data_ptr(), d.data_ptr(), code, rows, entries, dim,
+        _launch(d.get_device(), lib().nerf_embedding_bwd, 'nerf_embedding_bwd', index.data_ptr(), d.data_ptr(), code, rows, entries, dim,
                 ctx.scale, dtable.data_ptr(), _at(ws), n)
-        return dtable, None, None, None
+        return dtable, None, None
 
 
 class Embedding(nn.Module):
@@ -154,6 +163,11 @@ class Embedding(nn.Module):
 def rms_norm(x, weight, residual=None, eps=1e-6):
     """x / sqrt(mean(x^2) + eps) * weight over the last axis.  With `residual` (x's shape and type): (the norm of s, s) with
     s = x + residual rounded to x's type.  weight [dim]: x's type or float32."""
+    call = _NormFn.apply if _recorded(x, weight, residual) else _norm_fwd
+    return call(x, weight, residual, float(eps))
+
+
+def _norm_fwd(x, weight, residual, eps):
     code = _dtype(x, 'x')
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError('x must have a last axis of at least one column (got %s)' % (tuple(x.shape),))
@@ -167,12 +181,6 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
     if not eps >= 0:
         raise ValueError('eps must not be negative')
     device = _device('rms_norm', x, weight, residual)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        return _NormFn.apply(x, weight, residual, float(eps), code, device)
-    return _norm_fwd(x, weight, residual, float(eps), code, device)
-
-
-def _norm_fwd(x, weight, residual, eps, code, device):
     x, w = x.contiguous(), weight.contiguous()
     dim = x.shape[-1]
     y = torch.empty_like(x)
@@ -186,10 +194,10 @@ def _norm_fwd(x, weight, residual, eps, code, device):
 
 class _NormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps, code, device):
-        out = _norm_fwd(x, weight, residual, eps, code, device)
+    def forward(ctx, x, weight, residual, eps):
+        out = _norm_fwd(x, weight, residual, eps)
         ctx.save_for_backward(x if residual is None else out[1], weight)
-        ctx.eps, ctx.code, ctx.device = eps, code, device
+        ctx.eps = eps
         ctx.set_materialize_grads(False)
         return out
 
@@ -198,7 +206,7 @@ class _NormFn(torch.autograd.Function):
         total, weight = ctx.saved_tensors
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:      # only the sum was used
-            return dsum if need_x else None, torch.zeros_like(weight) if need_w else None, dsum if need_r else None, None, None, None
+            return dsum if need_x else None, torch.zeros_like(weight) if need_w else None, dsum if need_r else None, None
         s, w, d = total.contiguous(), weight.contiguous(), dy.contiguous()
         dim = s.shape[-1]
         rows = s.numel() // dim
@@ -207,9 +215,9 @@ class _NormFn(torch.autograd.Function):
         dw = torch.empty_like(w) if need_w else None
         n = lib().nerf_rmsnorm_bwd_workspace_bytes(rows, dim)
         ws = _workspace(n, 'nerf_rmsnorm_bwd', s)
-        _launch(ctx.device, lib().nerf_rmsnorm_bwd, 'nerf_rmsnorm_bwd', s.data_ptr(), w.data_ptr(), d.data_ptr(), _at(ds), ctx.code,
+        _launch(s.get_device(), lib().nerf_rmsnorm_bwd, 'nerf_rmsnorm_bwd', s.data_ptr(), w.data_ptr(), d.data_ptr(), _at(ds), DTYPES[s.dtype],
                 DTYPES[w.dtype], rows, dim, ctx.eps, _at(dx), _at(dw), _at(ws), n)
-        return dx if need_x else None, dw, dx if need_r else None, None, None, None
+        return dx if need_x else None, dw, dx if need_r else None, None
 
 
 class RMSNorm(nn.Module):
@@ -231,6 +239,12 @@ def gated_mlp(x, params, n_neurons, n_output_dims, activation='silu'):
     (FullyFusedMLP's layout), of x's type -- or float32 beside a 16-bit x: they are rounded on every call then, and their
     gradient is float32.  activation: silu, gelu (erf form) or relu.  The hidden values are held in x's type (float16: they
     overflow above 65504)."""
+    call = _GatedFn.apply if _recorded(x, params) else _gated_fwd
+    return call(x, params, n_neurons, n_output_dims, activation)
+
+
+def _gated_shape(x, params, n_neurons, n_output_dims, activation):
+    """Checks the arguments; (element type, n_in, n_neurons, n_out, activation) as the library takes them, and the device."""
     code = _dtype(x, 'x')
     if activation not in ACTIVATIONS:
         raise ValueError('activation must be one of %s (got %r)' % (', '.join(ACTIVATIONS), activation))
@@ -242,13 +256,14 @@ def gated_mlp(x, params, n_neurons, n_output_dims, activation='silu'):
     if params.dtype != x.dtype and params.dtype != torch.float32:
         raise TypeError('params must be %s or float32 (got %s)' % (x.dtype, params.dtype))
     device = _device('gated_mlp', x, params)
-    shape = (code, x.shape[-1], int(n_neurons), int(n_output_dims), ACTIVATIONS[activation], device)
-    if torch.is_grad_enabled() and (x.requires_grad or params.requires_grad):
-        return _GatedFn.apply(x, params, shape)
-    return _gated_fwd(x, params, shape, False)[0]
+    return code, x.shape[-1], int(n_neurons), int(n_output_dims), ACTIVATIONS[activation], device
 
 
-def _gated_fwd(x, params, shape, keep):
+def _gated_fwd(x, params, n_neurons, n_output_dims, activation):
+    return _gated_run(x, params, _gated_shape(x, params, n_neurons, n_output_dims, activation), False)[0]
+
+
+def _gated_run(x, params, shape, keep):
     code, n_in, neurons, n_out, act, device = shape
     x, w = _rows16(x), _rows16(params.to(x.dtype))
     rows = x.numel() // n_in
@@ -266,10 +281,10 @@ def _gated_fwd(x, params, shape, keep):
 
 class _GatedFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, params, shape):
-        y, saved = _gated_fwd(x, params, shape, True)
+    def forward(ctx, x, params, n_neurons, n_output_dims, activation):
+        ctx.shape = _gated_shape(x, params, n_neurons, n_output_dims, activation)
+        y, saved = _gated_run(x, params, ctx.shape, any(ctx.needs_input_grad))
         ctx.save_for_backward(x, params, saved)
-        ctx.shape = shape
         return y
 
     @_first_order
@@ -285,7 +300,7 @@ class _GatedFn(torch.autograd.Function):
         ws = _workspace(n, 'nerf_gated_mlp_bwd', x)
         _launch(device, lib().nerf_gated_mlp_bwd, 'nerf_gated_mlp_bwd', w.data_ptr(), x.data_ptr(), d.data_ptr(), _at(saved), code, rows,
                 n_in, neurons, n_out, act, _at(dx), _at(dparams), DTYPES[params.dtype], _at(ws), n)
-        return dx, dparams, None
+        return dx, dparams, None, None, None
 
 
 class GatedMLP(nn.Module):
