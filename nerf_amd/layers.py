@@ -26,7 +26,7 @@ ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 
 
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-_transforms = torch._C._functorch.peek_interpreter_stack
+_transforms, _tracing = torch._C._functorch.peek_interpreter_stack, torch._C._get_tracing_state
 
 
 def _launch(device, fn, what, *args):
@@ -79,10 +79,11 @@ def _at(t):
 
 def _recorded(a, b, c=None):
     """Whether a call goes through its autograd function: where a gradient will be asked for, and inside forward-mode differentiation
-    (whose tangents travel beside tensors that need no gradient) and torch.func's transforms.  The kernels write through raw pointers,
-    which neither of those sees: the function refuses them by name, as it has no `jvp` and no `setup_context`."""
+    (whose tangents travel beside tensors that need no gradient), torch.func's transforms and torch.jit.trace.  The kernels write
+    through raw pointers, which none of those sees.  The function refuses the first two by name, as it has no `jvp` and no
+    `setup_context`; a traced program records it as a call, with its checks of arguments."""
     return (torch.is_grad_enabled() and (a.requires_grad or b.requires_grad or (c is not None and c.requires_grad))
-            or forward_ad._current_level >= 0 or _transforms() is not None)
+            or forward_ad._current_level >= 0 or _transforms() is not None or _tracing() is not None)
 
 
 def _first_order(fn):

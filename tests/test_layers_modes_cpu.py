@@ -1,6 +1,6 @@
-"""nerf_amd.layers under the modes in which torch watches a call for more than its result -- forward-mode differentiation and
-torch.func's transforms -- without a GPU: a stand-in library computes what the entry points' header says of them with numpy, on
-the raw addresses that the functions pass, so that whatever reaches a caller has gone the same way as on the GPU."""
+"""nerf_amd.layers under the modes in which torch watches a call for more than its result -- forward-mode differentiation, torch.func's
+transforms, traced programs -- without a GPU: a stand-in library computes what the entry points' header says of them with numpy,
+on the raw addresses that the functions pass, so that whatever reaches a caller has gone the same way as on the GPU."""
 import ctypes as C
 
 import numpy as np
@@ -110,3 +110,18 @@ def test_function_transforms_are_refused(standin, name):
                         lambda: torch.func.functionalize(call)(x)):
         with pytest.raises(RuntimeError, match='setup_context'):
             transformed()
+
+
+@pytest.mark.filterwarnings('ignore')
+@pytest.mark.parametrize('leaf', [False, True])
+@pytest.mark.parametrize('name', list(CALLS))
+def test_a_traced_program_makes_the_call(standin, name, leaf):
+    """Also on other sizes than those it was traced with; and its arguments are checked on every run."""
+    call, plain = CALLS[name]
+    traced = torch.jit.trace(call, (randn(4, 8, seed=3).requires_grad_(leaf),), check_trace=False)
+    for rows in (4, 7):
+        x = randn(rows, 8, seed=4 + rows)
+        assert close(traced(x).detach(), plain(x))
+    for wrong in (randn(4, 8, seed=6).double(),) + (() if name == 'embedding' else (randn(4, 9, seed=6),)):
+        with pytest.raises(RuntimeError, match='must be'):
+            traced(wrong)
