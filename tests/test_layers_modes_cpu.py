@@ -1,5 +1,5 @@
 """nerf_amd.layers under the modes in which torch watches a call for more than its result -- forward-mode differentiation, torch.func's
-transforms, traced programs -- without a GPU: a stand-in library computes what the entry points' header says of them with numpy,
+transforms, traced programs, graphs of operations -- without a GPU: a stand-in library computes what the entry points' header says of them with numpy,
 on the raw addresses that the functions pass, so that whatever reaches a caller has gone the same way as on the GPU."""
 import ctypes as C
 
@@ -125,3 +125,18 @@ def test_a_traced_program_makes_the_call(standin, name, leaf):
     for wrong in (randn(4, 8, seed=6).double(),) + (() if name == 'embedding' else (randn(4, 9, seed=6),)):
         with pytest.raises(RuntimeError, match='must be'):
             traced(wrong)
+
+
+@pytest.mark.parametrize('mode', ['real', 'fake', 'symbolic'])
+@pytest.mark.parametrize('name', list(CALLS))
+def test_a_graph_of_operations_is_refused(standin, name, mode):
+    """Such a graph would hold the allocation of the result and not the launch.  (Other dispatch modes, which record nothing, may be on.)"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    call, plain = CALLS[name]
+    for leaf in (False, True):
+        x = randn(4, 8, seed=3).requires_grad_(leaf)
+        with pytest.raises(RuntimeError, match='make_fx|data pointer'):
+            make_fx(call, tracing_mode=mode)(x)
+        with FlopCounterMode(display=False):
+            assert close(call(x).detach(), plain(x))
