@@ -138,5 +138,7 @@ def test_a_graph_of_operations_is_refused(standin, name, mode):
         x = randn(4, 8, seed=3).requires_grad_(leaf)
         with pytest.raises(RuntimeError, match='make_fx|data pointer'):
             make_fx(call, tracing_mode=mode)(x)
+        with pytest.raises(RuntimeError, match='make_fx|data pointer'):
+            make_fx(call, tracing_mode=mode, pre_dispatch=True)(x)
         with FlopCounterMode(display=False):
             assert close(call(x).detach(), plain(x))
