@@ -337,6 +337,11 @@ class FusedAdam(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
+        for group in self.param_groups:     # (the kernels take raw pointers to floats; refused before any parameter is updated)
+            for p in group['params']:
+                if p.grad is not None and p.numel() > 0 and (p.dtype != torch.float32 or p.grad.dtype != torch.float32):
+                    raise TypeError('FusedAdam updates float32 parameters (got %s with a gradient of %s): keep a float32 master copy'
+                                    % (p.dtype, p.grad.dtype))
         flag = self.skip_flag
         self._skip_ptr = ptr(flag) if flag is not None else None
         self._stepped = []
@@ -382,9 +387,6 @@ class FusedAdam(torch.optim.Optimizer):
         b1, b2 = group['betas']
         if p.grad is None or p.numel() == 0:
             return
-        if p.dtype != torch.float32 or p.grad.dtype != torch.float32:     # (the kernels take raw pointers to floats)
-            raise TypeError('FusedAdam updates float32 parameters (got %s with a gradient of %s): keep a float32 master copy'
-                            % (p.dtype, p.grad.dtype))
         st = self.state[p]
         if not st:
             st['step'] = 0
