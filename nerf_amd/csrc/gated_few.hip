@@ -1,8 +1,8 @@
 // The gated block for few rows (up to 64): bound by reading the weights once.  No tile of rows is worth staging, so the weights go
 // from memory straight into the matrix cores' operand registers -- 16 weight rows by 32 k a fragment, 16 bytes a lane -- and the
-// waves of a workgroup split k: every wave takes each NW-th run of 128 k (256 bytes of each of the 16 rows), so a workgroup reads
-// whole stretches of its rows, and the waves' sums meet in LDS in wave order.  Two launches, h and y; y's tiles are too few for the chip where it is narrow: then
-// several workgroups share a tile's k and a third launch adds their sums.
+// waves of a workgroup split k: every wave takes each NW-th run of 64 to 256 k (run_steps), so a workgroup reads whole stretches of its
+// rows, and the waves' sums meet in LDS in wave order.  Two launches, h and y; y's tiles are too few for the chip where it is narrow:
+// then several workgroups share a tile's k and a third launch adds their sums.
 // Rows may start anywhere (16-byte loads at element alignment), so nothing is laid out first.  fp32 is cut into three bf16 parts on
 // the way (gated_mlp.hip says why).
 //
@@ -32,6 +32,9 @@ struct Few {
     int m, act;
 };
 
+// 32-k steps of a run -- what a wave has on its way at a time -- as the registers allow
+__host__ __device__ constexpr int run_steps(int parts, bool gate, int row_tiles) { return parts == 3 ? (gate ? 2 : 4) : gate || row_tiles > 1 ? 4 : 8; }
+
 // MT: 16-row tiles of x; NW: waves; kGate: both projections and h, or a plain product
 // FINE: h in two planes of 16 bits (kGate: p.plane says so)
 template <class T, int MT, int NW, bool kGate, bool FINE>
@@ -40,8 +43,7 @@ __global__ __launch_bounds__(NW * 64) void few_kernel(const T* __restrict__ w, c
     constexpr int P = Piece<T>::P, G = kGate ? 2 : 1, PX = kGate ? P : hidden_parts<T, FINE>();
     constexpr int XP = PX == 2 ? 2 : 1;     // planes of x
     typedef typename Piece<T>::E E;
-    // 32-k steps of a run -- what a wave has on its way at a time -- as the registers allow
-    constexpr int kRun = P == 3 ? (kGate ? 2 : 4) : kGate || MT > 1 ? 4 : 8;
+    constexpr int kRun = run_steps(P, kGate, MT);
     typedef typename Frag<E>::type frag;
     __shared__ f32x4 sums[NW][G][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
@@ -181,9 +183,12 @@ int64_t few_ld(int64_t f) { return (f + 31) / 32 * 32; }
 // are read once either way; x is read by every workgroup, as many 16-row tiles as it has.
 bool lays_x(int64_t m, int64_t k, int elem) { return m > 16 && k * elem % 16 != 0; }
 
-// y has few 16-column tiles: as many workgroups each as give every CU two, as long as each wave has a run of 128 k
-int parts_of(int64_t f, int64_t n) {
-    const int64_t want = 2 * kNumCU / ((n + 15) / 16), most = f / (128 * 8);
+// y has few 16-column tiles: as many workgroups each as give every CU two, and none that has no run (bf16, 1 row of 64 -> 2048 -> 512,
+// eight runs for one workgroup's waves: 9.3 us, shared by two 11.1; 9 rows of 64 -> 4000 -> 200 fp32, by four 12.4, by three 16.9).
+constexpr int kWaves = 8;
+int parts_of(int64_t m, int64_t f, int64_t n, int elem) {
+    const int64_t want = 2 * kNumCU / ((n + 15) / 16), run = 32 * run_steps(elem == 4 ? 3 : 1, false, m > 16 ? 2 : 1), runs = (f + run - 1) / run;
+    const int64_t most = (runs + kWaves - 1) / kWaves;
     return (int)(want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most);
 }
 
@@ -192,20 +197,20 @@ template <class T, int MT> int launch(const T* params, const T* x, int64_t m, in
     const int64_t plane = sizeof(T) == 2 && nerf_gated_fine(m, k, f, n) ? m * ldh : 0;
     Few up = {k, k, f, ldh, plane, (int)m, act};
     const Few down = {f, ldh, n, n, plane, (int)m, act};
-    const int parts = parts_of(f, n);
+    const int parts = parts_of(m, f, n, (int)sizeof(T));
     if (lays_x(m, k, (int)sizeof(T))) {
         up.ldx = few_ld(k);
         few_lay_kernel<T><<<(unsigned)ceil_div64(m * up.ldx, 256), 256, 0, st>>>(x, k, up.ldx, m * up.ldx, (T*)xl);
         x = (const T*)xl;
     }
-    few_kernel<T, MT, 8, true, false><<<(unsigned)(ldh / 16), 512, 0, st>>>(params, params + f * k, x, up, h, saved, nullptr);
+    few_kernel<T, MT, kWaves, true, false><<<(unsigned)(ldh / 16), kWaves * 64, 0, st>>>(params, params + f * k, x, up, h, saved, nullptr);
     const dim3 grid((unsigned)ceil_div64(n, 16), (unsigned)parts);
     const T* wd = params + 2 * f * k;
     if constexpr (sizeof(T) == 2) {
-        if (plane) few_kernel<T, MT, 8, false, true><<<grid, 512, 0, st>>>(wd, wd, h, down, y, nullptr, parts > 1 ? part : nullptr);
-        else few_kernel<T, MT, 8, false, false><<<grid, 512, 0, st>>>(wd, wd, h, down, y, nullptr, parts > 1 ? part : nullptr);
+        if (plane) few_kernel<T, MT, kWaves, false, true><<<grid, kWaves * 64, 0, st>>>(wd, wd, h, down, y, nullptr, parts > 1 ? part : nullptr);
+        else few_kernel<T, MT, kWaves, false, false><<<grid, kWaves * 64, 0, st>>>(wd, wd, h, down, y, nullptr, parts > 1 ? part : nullptr);
     } else {
-        few_kernel<T, MT, 8, false, false><<<grid, 512, 0, st>>>(wd, wd, h, down, y, nullptr, parts > 1 ? part : nullptr);
+        few_kernel<T, MT, kWaves, false, false><<<grid, kWaves * 64, 0, st>>>(wd, wd, h, down, y, nullptr, parts > 1 ? part : nullptr);
     }
     if (parts > 1) few_join_kernel<T><<<(unsigned)ceil_div64(m * n, 256), 256, 0, st>>>(part, parts, m * n, y);
     return nerf_launch_status("nerf_gated_mlp_fwd");
@@ -224,7 +229,7 @@ bool nerf_gated_few_ok(int64_t m) { return m <= 64; }
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 int64_t nerf_gated_few_bytes(int dtype, int64_t m, int64_t k, int64_t f, int64_t n) {
-    const int parts = parts_of(f, n), elem = nerf_dtype_bytes(dtype);
+    const int parts = parts_of(m, f, n, nerf_dtype_bytes(dtype)), elem = nerf_dtype_bytes(dtype);
     return up256(m * few_ld(f) * 4) +       // (of 16 bits: twice)
            (parts > 1 ? up256(parts * m * n * 4) : 0) + (lays_x(m, k, elem) ? m * few_ld(k) * elem : 0);
 }
@@ -232,7 +237,7 @@ int64_t nerf_gated_few_bytes(int dtype, int64_t m, int64_t k, int64_t f, int64_t
 int nerf_gated_few_fwd(const void* params, const void* x, int dtype, int64_t m, int64_t k, int64_t f, int64_t n, int act, void* y,
                        float* saved, void* ws, hipStream_t st) {
     const int64_t ldh = few_ld(f);
-    const int parts = parts_of(f, n);
+    const int parts = parts_of(m, f, n, nerf_dtype_bytes(dtype));
     char* part = (char*)ws + up256(m * ldh * 4);
     void* xl = part + (parts > 1 ? up256(parts * m * n * 4) : 0);
     int rc = 0;
