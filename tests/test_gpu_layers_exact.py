@@ -43,3 +43,45 @@ def test_a_few_thousand_values_are_as_exact_as_their_rounding(dtype, rows, k, f,
     for got, w, what in ((y.detach(), want[0], 'y'), (gated_mlp(x, p, f, n_out), want[0], 'y alone'), (dx, want[1], 'dx'),
                          (dp, torch.cat([q.reshape(-1) for q in want[2:]]), 'dparams')):
         assert rms(got.double() - w) <= 1.15 * rms(w.to(t).double() - w), what
+
+
+# float32 products are those of three bf16 parts of each side, six of nine (gated_mlp.hip).  Leaving one of the six out of one of the
+# block's six kinds of product makes some result's relative root-mean-square error 2.4e-6 or more (test_layers_exact_cpu.py emulates that).
+# With all of them it is made of roundings: one of a running sum is off by 2^-24 / sqrt(3) of it at the root mean square, and a sum in c
+# steps, whose running value grows with the root of the step, by sqrt(c / 2) of those; a matrix instruction takes 16 or 32 of k, the
+# low orders' steps are 2^-8 as large, so the longest sums here (4001 rows or 2667 hidden values, in splits) have c < 250: 3.8e-7.
+# A result carries up to four such sums (g and u, dh, its own): 2^-20 = 9.5e-7 holds them and is less than half of what a lost product makes.
+F32_RMS = 2.0 ** -20
+F32_SHAPES = {
+    'few rows': (40, 100, 130, 90),
+    'narrow, one launch each way': (1000, 40, 100, 30),
+    'narrow, two launches each way': (1000, 51, 241, 51),
+    'wide, g, u, y and dh in one split': (1200, 72, 96, 80),
+    'wide, splits': (700, 100, 130, 90),
+    'wide, 256 tiles': (4001, 1001, 2667, 1001),
+}
+
+
+def relative_rms(got, want):
+    return [rms(a.double() - b) / rms(b) for a, b in zip(got, want)]
+
+
+def as_exact_as_float32(got, want):
+    return max(relative_rms(got, want)) <= F32_RMS
+
+
+def parted(dp, k, f, n_out):
+    return [q.view(s) for q, s in zip(torch.split(dp, (f * k, f * k, n_out * f)), ((f, k), (f, k), (n_out, f)))]
+
+
+@pytest.mark.parametrize('what', list(F32_SHAPES))
+def test_float32_loses_none_of_its_products(what):
+    from nerf_amd.layers import gated_mlp
+    rows, k, f, n_out = F32_SHAPES[what]
+    x, p, dy = gated_inputs(rows, k, f, n_out, torch.float32, seed=29)
+    xr, pr = x.clone().requires_grad_(True), p.clone().requires_grad_(True)
+    y = gated_mlp(xr, pr, f, n_out)
+    dx, dp = torch.autograd.grad(y, (xr, pr), dy)
+    want = gated64(x, p, f, n_out, dy)
+    assert as_exact_as_float32([y.detach(), dx] + parted(dp, k, f, n_out), want), relative_rms([y.detach(), dx] + parted(dp, k, f, n_out), want)
+    assert as_exact_as_float32([gated_mlp(x, p, f, n_out)], want)
