@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_gpu_layers import TYPES, gated_inputs, gated_reference, within
+from test_gpu_layers import F32, TYPES, gated_inputs, gated_reference, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,39 @@ def test_few_rows_share_a_tile_among_workgroups(dtype, rows, k, f, n_out):
     assert (ws[n:] == 0x5a).all() and (y[size:] == 0x5a).all()
     wy, by = gated_reference(x, p, f, n_out, dy, 'silu', t)[:2]
     within(y[:size].view(t).view(rows, n_out), wy, by, 'y')
+
+
+# Sort of the table's gradient: tiles of 1024 positions, of 4096 above 2^20 of them; their counts are summed in a launch of their own above 48
+# tiles; a pass for every 8 bits of the table's size.
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('rows,entries,dim', [
+    (60000, 70000, 5), (49152, 300, 3), (49153, 300, 3), (70000, 70000, 5), (1048576, 300, 1), (1048577, 256, 2), (1100000, 1000, 3),
+    (2200000, 20, 1), (1200000, 70000, 2), (100000, 200, 9), (4096, 70000, 4), (4097, 300, 4)])
+def test_every_position_reaches_its_entry(dtype, rows, entries, dim):
+    """Gradients of small whole numbers: fp32 sums of them are exact below 2^24 in any order, so the table's gradient has to be the whole
+    numbers' sum, rounded once -- for the guarded entry point with the workspace it asks for."""
+    from nerf_amd._lib import lib, ptr
+    t, code, L = TYPES[dtype], CODES[dtype], lib()
+    g = torch.Generator().manual_seed(rows + entries)
+    index = torch.randint(-2, entries + 2, (rows,), generator=g)        # some outside the table, on both sides
+    index[rows // 2:rows // 2 + 5000] = entries // 3                    # and a long stretch of one entry
+    whole = torch.randint(-9, 10, (rows, dim), generator=g)
+    index, dy = index.cuda(), whole.to(t).cuda()
+    ok = (index >= 0) & (index < entries)
+    want = torch.zeros(entries, dim, dtype=torch.int64).index_add_(0, index.cpu()[ok.cpu()], whole[ok.cpu()])
+    assert int(want.abs().max()) < 1 << 24
+    n, size = L.nerf_embedding_bwd_workspace_bytes(code, entries, dim, rows), entries * dim * t.itemsize
+    ws, out = guarded(n), guarded(size)
+    assert L.nerf_embedding_bwd(ptr(index), ptr(dy), code, rows, entries, dim, 1.0, ptr(out), ptr(ws), n, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert (ws[n:] == 0x5a).all() and (out[size:] == 0x5a).all()
+    assert torch.equal(out[:size].view(t).view(entries, dim), want.float().to(t).cuda())
+    # and through the layer, with values whose sums do round: the same bits twice
+    from nerf_amd.layers import embedding
+    table, values = randn(entries, dim, seed=1).to(t).requires_grad_(True), randn(rows, dim, seed=2).to(t)
+    once, again = (torch.autograd.grad(embedding(index, table, 0.7), table, values)[0] for _ in range(2))
+    assert torch.equal(once, again)
+    exact, size_of = (torch.zeros(entries, dim, dtype=torch.float64, device='cuda').index_add_(0, index[ok], v.double()[ok]) * 0.7
+                      for v in (values, values.abs()))
+    count = torch.bincount(index[ok], minlength=entries).double()[:, None]
+    within(once, exact, (count + 8) * F32 * size_of, 'table gradient')      # (8: 0.7 in fp32 and its product among them)
