@@ -64,3 +64,25 @@ def test_every_position_reaches_its_entry(dtype, rows, entries, dim):
                       for v in (values, values.abs()))
     count = torch.bincount(index[ok], minlength=entries).double()[:, None]
     within(once, exact, (count + 8) * F32 * size_of, 'table gradient')      # (8: 0.7 in fp32 and its product among them)
+
+
+# The wide block in 256 x 256 tiles: every product of it, in whole tiles and in ragged ones.
+@pytest.mark.parametrize('dtype,rows,k,f,n_out,act', [
+    ('bf16', 3000, 1500, 3000, 2900, 'silu'), ('f16', 3000, 1500, 3000, 2900, 'gelu'), ('bf16', 4096, 4096, 4096, 4096, 'relu'),
+    ('f16', 4096, 4096, 4096, 4096, 'silu'), ('f32', 4001, 1001, 2667, 1001, 'gelu'), ('f32', 4096, 2048, 4096, 2048, 'silu')])
+def test_large_tiles(dtype, rows, k, f, n_out, act):
+    from nerf_amd.layers import gated_mlp
+    from test_gpu_layers_exact import F32_RMS, rms
+    t = TYPES[dtype]
+    x, p, dy = gated_inputs(rows, k, f, n_out, t, seed=70)
+    xr, pr = x.clone().requires_grad_(True), p.clone().requires_grad_(True)
+    y = gated_mlp(xr, pr, f, n_out, activation=act)
+    dx, dp = torch.autograd.grad(y, (xr, pr), dy)
+    alone = gated_mlp(x, p, f, n_out, activation=act)
+    wy, by, wdx, bdx, wdp, bdp = gated_reference(x, p, f, n_out, dy, act, t)
+    for got, want, bound, what in ((y.detach(), wy, by, 'y'), (alone, wy, by, 'y alone'), (dx, wdx, bdx, 'dx'), (dp, wdp, bdp, 'dparams')):
+        within(got, want, bound, what)
+        # as a whole: 16 bits, the result's own rounding and one of hidden values of the same size (a ratio of 1.41; 1.5 leaves
+        # room for fp32); float32: what test_gpu_layers_exact.py derives
+        off = rms(got.double() - want)
+        assert off <= (F32_RMS * rms(want) if t == torch.float32 else 1.5 * rms(want.to(t).double() - want)), (what, off)
