@@ -443,6 +443,7 @@ int nerf_rmsnorm_bwd(const void* sum /*[n_rows,dim]*/, const void* weight, const
  * n_rows <= 2^26, widths <= 65536. */
 int64_t nerf_gated_mlp_saved_floats(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out); /* < 0: error */
 int64_t nerf_gated_mlp_fwd_workspace_bytes(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out);
+int64_t nerf_gated_mlp_alone_workspace_bytes(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out); /* without `saved` */
 int64_t nerf_gated_mlp_bwd_workspace_bytes(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out);
 int nerf_gated_mlp_fwd(const void* params, const void* x /*[n_rows,n_in]*/, int dtype, int64_t n_rows, int64_t n_in,
                        int64_t n_neurons, int64_t n_out, int activation, void* y /*[n_rows,n_out]*/, float* saved,

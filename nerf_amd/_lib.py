@@ -116,6 +116,7 @@ SIGNATURES = {
     'nerf_rmsnorm_bwd': (_I, [_P, _P, _P, _P, _I, _I, _I64, _I64, _F, _P, _P, _P, _I64, _P]),
     'nerf_gated_mlp_saved_floats': (_I64, [_I, _I64, _I64, _I64, _I64]),
     'nerf_gated_mlp_fwd_workspace_bytes': (_I64, [_I, _I64, _I64, _I64, _I64]),
+    'nerf_gated_mlp_alone_workspace_bytes': (_I64, [_I, _I64, _I64, _I64, _I64]),
     'nerf_gated_mlp_bwd_workspace_bytes': (_I64, [_I, _I64, _I64, _I64, _I64]),
     'nerf_gated_mlp_fwd': (_I, [_P, _P, _I, _I64, _I64, _I64, _I64, _I, _P, _P, _P, _I64, _P]),
     'nerf_gated_mlp_bwd': (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I, _P, _P, _I, _P, _I64, _P]),

@@ -801,8 +801,8 @@ template <class F> int by_type(int dtype, int hidden, F&& f) {
 // The narrow kernels where they apply -- the forward one only where no backward pass needs g and u kept.
 bool narrow_fwd(const Shape& s, int dtype, bool keep) { return !keep && nerf_gated_narrow_fwd_ok(dtype, s.m, s.k, s.f, s.n); }
 bool narrow_bwd(const Shape& s, int dtype) { return nerf_gated_narrow_bwd_ok(dtype, s.k, s.f, s.n); }
-int64_t fwd_bytes(const Shape& s, int dtype) {
-    if (narrow_fwd(s, dtype, !narrow_bwd(s, dtype))) return 0;
+int64_t fwd_bytes(const Shape& s, int dtype, bool keep) {
+    if (narrow_fwd(s, dtype, keep && !narrow_bwd(s, dtype))) return 0;
     return nerf_gated_few_ok(s.m) ? nerf_gated_few_bytes(dtype, s.m, s.k, s.f, s.n) : FwdSpace(s).bytes;
 }
 int64_t bwd_bytes(const Shape& s, int dtype) { return narrow_bwd(s, dtype) ? nerf_gated_narrow_bwd_bytes(dtype, s.m, s.k, s.f, s.n) : BwdSpace(s).bytes; }
@@ -828,7 +828,12 @@ extern "C" int64_t nerf_gated_mlp_saved_floats(int dtype, int64_t n_rows, int64_
 
 extern "C" int64_t nerf_gated_mlp_fwd_workspace_bytes(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out) {
     if (bad_shape(dtype, n_rows, n_in, n_neurons, n_out, NERF_ACT_SILU)) return -1;
-    return fwd_bytes(Shape(dtype, n_rows, n_in, n_neurons, n_out), dtype);
+    return fwd_bytes(Shape(dtype, n_rows, n_in, n_neurons, n_out), dtype, true);
+}
+
+extern "C" int64_t nerf_gated_mlp_alone_workspace_bytes(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out) {
+    if (bad_shape(dtype, n_rows, n_in, n_neurons, n_out, NERF_ACT_SILU)) return -1;
+    return fwd_bytes(Shape(dtype, n_rows, n_in, n_neurons, n_out), dtype, false);
 }
 
 extern "C" int64_t nerf_gated_mlp_bwd_workspace_bytes(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out) {
@@ -843,7 +848,7 @@ extern "C" int nerf_gated_mlp_fwd(const void* params, const void* x, int dtype, 
     NERF_REQUIRE(!bad, bad);
     if (n_rows == 0) return 0;
     const Shape s(dtype, n_rows, n_in, n_neurons, n_out);
-    const int64_t need = fwd_bytes(s, dtype);
+    const int64_t need = fwd_bytes(s, dtype, saved != nullptr);
     NERF_REQUIRE(params && x && y && (workspace || need == 0), "null pointer");
     NERF_REQUIRE(nerf_aligned(params, 16) && nerf_aligned(x, 16) && nerf_aligned(workspace, 16), "params, x and workspace must be 16-byte aligned");
     NERF_REQUIRE(workspace_bytes >= need, "workspace too small");

@@ -276,7 +276,7 @@ def _gated_run(x, params, shape, keep):
     rows = x.numel() // n_in
     y = x.new_empty(x.shape[:-1] + (n_out,))
     saved = None
-    n = lib().nerf_gated_mlp_fwd_workspace_bytes(code, rows, n_in, neurons, n_out)
+    n = (lib().nerf_gated_mlp_fwd_workspace_bytes if keep else lib().nerf_gated_mlp_alone_workspace_bytes)(code, rows, n_in, neurons, n_out)
     ws = _workspace(n, 'nerf_gated_mlp_fwd', x)
     if keep:
         kept = lib().nerf_gated_mlp_saved_floats(code, rows, n_in, neurons, n_out)

@@ -86,3 +86,21 @@ def test_large_tiles(dtype, rows, k, f, n_out, act):
         # room for fp32); float32: what test_gpu_layers_exact.py derives
         off = rms(got.double() - want)
         assert off <= (F32_RMS * rms(want) if t == torch.float32 else 1.5 * rms(want.to(t).double() - want)), (what, off)
+
+
+# (weights of 32 hidden values in LDS: 16 KiB beside more than 64 columns of x, and 8 or 4 KiB for those of y: 192 and 256 hidden values in 160 KiB)
+@pytest.mark.parametrize('dtype,k,f,n_out', [('bf16', 100, 192, 100), ('bf16', 100, 256, 64), ('f16', 128, 128, 40), ('f32', 50, 200, 60)])
+def test_a_narrow_block_alone_allocates_its_result_only(dtype, k, f, n_out):
+    from nerf_amd.layers import gated_mlp
+    t, rows = TYPES[dtype], 30000
+    x, p, dy = gated_inputs(rows, k, f, n_out, t, seed=80)
+    gated_mlp(x[:65], p, f, n_out)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = gated_mlp(x, p, f, n_out)
+    assert torch.cuda.max_memory_allocated() - before <= (y.numel() * t.itemsize + 511) // 512 * 512      # (the allocator's step)
+    wy, by = gated_reference(x, p, f, n_out, dy, 'silu', t)[:2]
+    within(y, wy, by, 'y')
+    kept = gated_mlp(x, p.clone().requires_grad_(True), f, n_out).detach()
+    within(kept, wy, by, 'y with a backward pass to follow')
