@@ -55,6 +55,28 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float* lds)
     return s;
 }
 
+// the largest magnitude of a row, given to all its threads (NaNs aside: the sums show them)
+template <int TPR> __device__ __forceinline__ float row_max(float v, float* lds) {
+#pragma unroll
+    for (int o = (TPR < 64 ? TPR : 64) / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    if constexpr (TPR > 64) {
+        constexpr int kWaves = TPR / 64;
+        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+        __syncthreads();
+        const int w0 = (threadIdx.x / TPR) * kWaves;
+        for (int i = 0; i < kWaves; ++i) v = fmaxf(v, lds[w0 + i]);
+        __syncthreads();
+    }
+    return v;
+}
+// Rows whose squares leave fp32's range -- a sum above 2^120, or below 2^-80 with no eps to speak of beside it -- are scaled by the
+// power of two that takes the larger of their largest value and eps's root to [1/2, 1), and eps by its square: y is the same.
+__device__ __forceinline__ bool out_of_range(float ss, float eps) { return !(ss <= 0x1p120f && (ss >= 0x1p-80f || eps >= 0x1p-100f)); }
+__device__ __forceinline__ int row_exponent(float largest, float eps) {
+    const float v = fmaxf(largest, sqrtf(eps));
+    return v > 0.f && v < __builtin_inff() ? __builtin_amdgcn_frexp_expf(v) : 0;        // (0 / 0 and infinities stay what they are)
+}
+
 // two sums at once, one barrier: `lds` (32 floats) must not be the one of the call before (two in turn)
 template <int TPR> __device__ __forceinline__ void row_sum2(float& a, float& b, float* lds) {
     if constexpr (TPR <= 64) {
@@ -115,7 +137,27 @@ __global__ __launch_bounds__(RowThreads<TPR>::kBlock) void rmsnorm_fwd_kernel(co
 #pragma unroll
         for (int i = 0; i < N; ++i) ss = fmaf(s[j][i], s[j][i], ss);
     }
-    const float r = 1.0f / sqrtf(row_sum<TPR>(ss, lds) / (float)dim + eps);
+    ss = row_sum<TPR>(ss, lds);
+    float scaled_eps = eps;
+    if (out_of_range(ss, eps)) {        // (the same for all threads of the row)
+        float largest = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) largest = fmaxf(largest, fabsf(s[j][i]));
+        const int e = row_exponent(row_max<TPR>(largest, lds), eps);
+        ss = 0.f;
+        scaled_eps = ldexpf(eps, -2 * e);
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                s[j][i] = ldexpf(s[j][i], -e);
+                ss = fmaf(s[j][i], s[j][i], ss);
+            }
+        ss = row_sum<TPR>(ss, lds);
+    }
+    const float r = 1.0f / sqrtf(ss / (float)dim + scaled_eps);
     if (!live) continue;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -148,9 +190,22 @@ __global__ __launch_bounds__(1024) void rmsnorm_fwd_long_kernel(const T* __restr
         }
         ss = fmaf(v, v, ss);
     }
-    const float r = 1.0f / sqrtf(row_sum<1024>(ss, lds) / (float)dim + eps);
-    for (int64_t c = threadIdx.x; c < dim; c += 1024)       // (a thread reads back only what it wrote itself)
-        y[at + c] = (T)((float)(RES ? sum[at + c] : x[at + c]) * r * (float)w[c]);
+    ss = row_sum<1024>(ss, lds);
+    const T* s_ = RES ? sum : x;        // (a thread reads back only what it wrote itself)
+    int e = 0;
+    if (out_of_range(ss, eps)) {
+        float largest = 0.f;
+        for (int64_t c = threadIdx.x; c < dim; c += 1024) largest = fmaxf(largest, fabsf((float)s_[at + c]));
+        e = row_exponent(row_max<1024>(largest, lds), eps);
+        ss = 0.f;
+        for (int64_t c = threadIdx.x; c < dim; c += 1024) {
+            const float v = ldexpf((float)s_[at + c], -e);
+            ss = fmaf(v, v, ss);
+        }
+        ss = row_sum<1024>(ss, lds);
+    }
+    const float r = 1.0f / sqrtf(ss / (float)dim + ldexpf(eps, -2 * e));
+    for (int64_t c = threadIdx.x; c < dim; c += 1024) y[at + c] = (T)(ldexpf((float)s_[at + c], -e) * r * (float)w[c]);
     }
 }
 
@@ -161,7 +216,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::kBlock) void rmsnorm_bwd_kernel(co
                                                                               T* __restrict__ dx, float* __restrict__ part,
                                                                               W* __restrict__ dweight) {
     constexpr int N = Vec16<T>::N, kRows = RowThreads<TPR>::kRows;
-    __shared__ float lds[64];
+    __shared__ float lds[112];      // two sums in turn; those of a scaled row, and its largest value
     extern __shared__ float dwl[];      // [4][dim]: the waves' sums (kRows > 1 only)
     const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
     float dw[NV][N], wv[NV][N];
@@ -206,8 +261,27 @@ __global__ __launch_bounds__(RowThreads<TPR>::kBlock) void rmsnorm_bwd_kernel(co
         }
         fetch(row + (int64_t)gridDim.x * kRows);
         row_sum2<TPR>(ss, sd, lds + 32 * turn);
-        const float r = 1.0f / sqrtf(ss / (float)dim + eps);
-        const float c = sd * r / (float)dim;
+        int p = 0;
+        if (out_of_range(ss, eps)) {        // (the same for all threads of the row)
+            float largest = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) largest = fmaxf(largest, fabsf(s[j][i]));
+            p = row_exponent(row_max<TPR>(largest, lds + 96), eps);
+            ss = sd = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    s[j][i] = ldexpf(s[j][i], -p);
+                    ss = fmaf(s[j][i], s[j][i], ss);
+                    sd = fmaf(d[j][i] * wv[j][i], s[j][i], sd);
+                }
+            row_sum2<TPR>(ss, sd, lds + 64);
+        }
+        const float r = 1.0f / sqrtf(ss / (float)dim + ldexpf(eps, -2 * p));        // (of the scaled row)
+        const float c = sd * r / (float)dim, rx = ldexpf(r, -p);
         if (live) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -218,7 +292,7 @@ __global__ __launch_bounds__(RowThreads<TPR>::kBlock) void rmsnorm_bwd_kernel(co
                 for (int i = 0; i < N; ++i) {
                     const float n = s[j][i] * r;
                     dw[j][i] = fmaf(d[j][i], n, dw[j][i]);
-                    const float ds = (d[j][i] * wv[j][i] - n * c) * r;
+                    const float ds = (d[j][i] * wv[j][i] - n * c) * rx;
                     o[i] = dsum ? ds + (float)e[j].v[i] : ds;
                 }
                 if (dx) store_cols<WHOLE>(dx + at, col, dim, o);
@@ -276,12 +350,26 @@ __global__ __launch_bounds__(1024) void rmsnorm_bwd_long_kernel(const T* __restr
         }
         ss = row_sum<1024>(ss, lds);
         sd = row_sum<1024>(sd, lds);
-        const float r = 1.0f / sqrtf(ss / (float)dim + eps);
-        const float k = sd * r / (float)dim;
+        int p = 0;
+        if (out_of_range(ss, eps)) {
+            float largest = 0.f;
+            for (int64_t c = threadIdx.x; c < dim; c += 1024) largest = fmaxf(largest, fabsf((float)s_[at + c]));
+            p = row_exponent(row_max<1024>(largest, lds), eps);
+            ss = sd = 0.f;
+            for (int64_t c = threadIdx.x; c < dim; c += 1024) {
+                const float s = ldexpf((float)s_[at + c], -p);
+                ss = fmaf(s, s, ss);
+                sd = fmaf((float)dy[at + c] * (float)w[c], s, sd);
+            }
+            ss = row_sum<1024>(ss, lds);
+            sd = row_sum<1024>(sd, lds);
+        }
+        const float r = 1.0f / sqrtf(ss / (float)dim + ldexpf(eps, -2 * p));        // (of the scaled row)
+        const float k = sd * r / (float)dim, rx = ldexpf(r, -p);
         for (int64_t c = threadIdx.x; c < dim; c += 1024) {
-            const float n = (float)s_[at + c] * r, d = (float)dy[at + c];
+            const float n = ldexpf((float)s_[at + c], -p) * r, d = (float)dy[at + c];
             mine[c] = fmaf(d, n, mine[c]);
-            const float ds = (d * (float)w[c] - n * k) * r;
+            const float ds = (d * (float)w[c] - n * k) * rx;
             if (dx) dx[at + c] = (T)(dsum ? ds + (float)dsum[at + c] : ds);
         }
     }
