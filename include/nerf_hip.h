@@ -416,8 +416,8 @@ int nerf_cum_weights_thresh(const float* weights, int64_t n_rays, int n_samples,
  * safe: a row of zeros, and no gradient.  n_entries, n_rows < 2^31, dim <= 2^20. */
 int nerf_embedding_fwd(const void* table /*[n_entries,dim]*/, int dtype, int64_t n_entries, int64_t dim,
                        const int64_t* index /*[n_rows]*/, int64_t n_rows, float scale, void* out /*[n_rows,dim]*/, void* stream);
-/* dtable[v] = scale * sum over i with index[i] == v of dout[i], i ascending; every row of dtable is WRITTEN (zeros where no
- * index points). */
+/* dtable[v] = scale * sum over i with index[i] == v of dout[i], in an order that the sizes and `index` fix; every row of dtable is
+ * WRITTEN (zeros where no index points). */
 int64_t nerf_embedding_bwd_workspace_bytes(int dtype, int64_t n_entries, int64_t dim, int64_t n_rows); /* < 0: error */
 int nerf_embedding_bwd(const int64_t* index, const void* dout /*[n_rows,dim]*/, int dtype, int64_t n_rows, int64_t n_entries,
                        int64_t dim, float scale, void* dtable /*[n_entries,dim]*/, void* workspace, int64_t workspace_bytes,
@@ -438,7 +438,8 @@ int nerf_rmsnorm_bwd(const void* sum /*[n_rows,dim]*/, const void* weight, const
  * [n_out,n_neurons], row-major, one after another (the layout of nerf_mlp_fwd's layers).  params, x, dy and workspaces start at
  * multiples of 16 bytes.  saved (nullable: no backward pass will follow): nerf_gated_mlp_saved_floats floats that the forward
  * pass fills for the backward pass (x Wg^T and x Wu^T; none where that one computes them again).  16 bits: the hidden values
- * h = act(g) * u are held in dtype (in two parts of it where rows or weights are few); fp16 ones overflow to infinity above 65504.
+ * h = act(g) * u are held in dtype, in two parts of it where rows or weights are few, so that a row may be held more exactly alone
+ * than among others; fp16 ones overflow to infinity above 65504.
  * fp32: products are exact to 2^-24 of a term.  Where the formula gives an infinity, a NaN may come out.
  * n_rows <= 2^26, widths <= 65536. */
 int64_t nerf_gated_mlp_saved_floats(int dtype, int64_t n_rows, int64_t n_in, int64_t n_neurons, int64_t n_out); /* < 0: error */

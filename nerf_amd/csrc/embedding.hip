@@ -1,21 +1,21 @@
 // Row lookup with scaling, and its gradient by sorted indices.
 //
 //   y[i] = round(scale * table[index[i]])                                   (an index outside the table: a row of zeros)
-//   dtable[v] = round(scale * sum over i with index[i] = v, i ascending, of dy[i])      (rows nobody looked up: zeros)
+//   dtable[v] = round(scale * sum over i with index[i] = v of dy[i])                        (rows nobody looked up: zeros)
 //
 // Backward.  Adding rows into the table with atomics gives other bits every time and serialises on the rows that many positions
 // share (every sample of a ray looks up the same image's code).  Here the positions are sorted by index instead -- a stable
 // radix sort of (index, position) pairs, 8 bits a pass, as many passes as the table's size has bytes, in one launch where a
-// workgroup holds them all -- and every stretch of equal indices is added up in ascending position order: the order, and so
-// every bit, is the same each time.
+// workgroup holds them all -- and every stretch of equal indices is added up in an order that sizes and indices alone decide (the
+// positions of a share ascending, then the shares by stripes, below): every bit is the same each time.
 //   A GROUP of lanes owns one 16-byte column piece per lane and walks its share of the sorted positions, keeping the running row in
 // registers.  A stretch that lies within one share is finished there; one that crosses shares leaves its partial rows (fp32)
 // in the workspace -- a share has at most two: the stretch it starts in the middle of and the one it ends in the middle of --
-// and a second launch adds those up in share order.  Rows that nobody looked up have to be zeros: the whole table is cleared by
+// and a second launch adds those up: a workgroup's threads each every so many-th share, ascending, then the threads' sums.  Rows that nobody looked up have to be zeros: the whole table is cleared by
 // spare workgroups of the sort's launches, which leave most of the chip idle.
 //
 // Measured.  Forward, bound by HBM writes: 786432 rows of 48 fp32 in 33 to 35 us (4.5 TB/s), 32768 of 1000 bf16 in 26 us.  Backward, the same
-// sizes: the sort 21 us in one pass and 30 us in two (50000 entries; with 100 MB of table cleared meanwhile), sums 45 and 33 us (3.3 and
+// sizes: the sort 21 us in one pass and 33 us in two (50000 entries; with 100 MB of table cleared meanwhile), sums 45 and 33 us (3.3 and
 // 2.0 TB/s of rows gathered by position), joins 9 and 23 us (the longest stretch: a workgroup for 256 of its columns).
 #include "layers_common.h"
 

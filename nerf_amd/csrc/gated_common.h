@@ -141,7 +141,8 @@ static inline int64_t saved_floats(int64_t rows, int64_t neurons) { return (neur
 // times of many.  Emulated in 64 bits with hidden values of normal inputs, 150 blocks each, by the smallest of y, h and dx: of 300 values
 // (or 200 weights) one block in 5 had an output 1.5 times as far off as one whose hidden values are not rounded, of 1024 one in
 // 15 to 25, of 2048 one in 20 to 75, of 4096 (or 3000 weights) at most one in 100.  What two parts cost, for calls of
-// 2048 to 4095 values: bf16 1 row of 2048 -> 8192 -> 2048 24.8 us, in one part 22.6; 3 of 1365 -> 4000 -> 1365 20.9 | 19.6; 90 of 40 -> 2000 -> 40 21.1 | 20.8.
+// 2048 to 4095 values: bf16 1 row of 2048 -> 8192 -> 2048 24.8 us, in one part 22.6; 3 of 1365 -> 4000 -> 1365 20.9 | 19.6; 90 of 40 -> 2000 -> 40 21.1 | 20.8;
+// 37 of 64 -> 3000 -> 1536, where every row tile reads both parts of h, 25.4 | 18.2.
 static inline bool nerf_gated_fine(int64_t m, int64_t k, int64_t f, int64_t n) {
     const int64_t least = k < f ? (k < n ? k : n) : (f < n ? f : n);
     return m * least < 4096 || (2 * k + n) * f <= 4096;

@@ -6,8 +6,8 @@
 // Rows may start anywhere (16-byte loads at element alignment), so nothing is laid out first.  fp32 is cut into three bf16 parts on
 // the way (gated_mlp.hip says why).
 //
-// Measured: 1 row, 2048 -> 8192 -> 2048 bf16: h 13.7 us (67 MB of weights at 4.9 TB/s), y 8.2 + 2.3 us (33 MB, with its join);
-// 37 rows, 1536 -> 4000 -> 1536 fp16: 11.1 and 11.3 + 3.0 us (25 and 12 MB: by the latency of the few turns a wave has; with four row
+// Measured: 1 row, 2048 -> 8192 -> 2048 bf16: h 14.3 us (67 MB of weights at 4.7 TB/s), y 10.8 + 3.0 us (33 MB, h in two parts, with its join);
+// 37 rows, 1536 -> 4000 -> 1536 fp16: 10.7 and 10.1 + 2.7 us (25 and 12 MB: by the latency of the few turns a wave has; with four row
 // tiles in place of three 1.2 us more).  Rows and weights sent for together, all row tiles at a time: 27 us in place of 24 for the one
 // row, for want of registers.
 #include <type_traits>

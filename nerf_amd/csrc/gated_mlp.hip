@@ -14,9 +14,9 @@
 // Roundings: h, dg and du are rounded to the element type (fp32: cut into three bf16) because the matrix cores read them so;
 // g and u are kept in fp32 between the passes, so that the activation's derivative is taken of what the forward pass had.
 //
-// Measured, 8192 rows, 2048 -> 8192 -> 2048 bf16 (a large library product: 1.2 to 1.5 PFLOP/s at these shapes): g, u and h 571 us (0.96
-// PFLOP/s with 537 MB of g and u stored), y 245 us (1.12), dh with dg, du and h again 411 us (0.67: reads g and u), dx 462 us (1.19), the
-// weights' gradients 373 us each on average (1.11).  fp32, 4001 rows, 1001 -> 2667 -> 1001: 333, 125, 251, 240 and 199 us each (0.7 to 1.1
+// Measured, 8192 rows, 2048 -> 8192 -> 2048 bf16 (a large library product: 1.2 to 1.5 PFLOP/s at these shapes): g, u and h 567 us (0.97
+// PFLOP/s with 537 MB of g and u stored), y 245 us (1.12), dh with dg, du and h again 411 us (0.67: reads g and u), dx 467 us (1.18), the
+// weights' gradients 382 us each on average (1.08).  fp32, 4001 rows, 1001 -> 2667 -> 1001: 335, 125, 254, 238 and 202 us each (0.7 to 1.1
 // PFLOP/s of bf16 products), laying out 35 us and joins 18 us each.
 #include <type_traits>
 

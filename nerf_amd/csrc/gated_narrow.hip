@@ -17,7 +17,7 @@
 // products.
 //
 // Measured, 786432 rows, 64 -> 128 -> 64 bf16: forward 60 us (0.64 PFLOP/s, 3.3 TB/s; the matrix cores share their issue slots with the
-// activations), backward 182 to 200 + 9 us (0.5 PFLOP/s with what it computes again; a tile's products, transposed reads and
+// activations), backward 182 to 205 + 9 us by card (0.5 PFLOP/s with what it computes again; a tile's products, transposed reads and
 // activations follow one another in the one or two waves of a SIMD).  fp32, 65799 rows of the same: 37 and 104 + 6 us.
 #include <type_traits>
 

@@ -11,8 +11,9 @@
 // its row groups in pairs; one partial row per workgroup goes to the workspace, and a second launch adds those in a fixed order: no
 // atomics, the same bits every time.
 //
-// Measured, with a residual: 786432 x 64 fp32 forward 135 us (6.0 TB/s, some of it from the last-level cache), backward 162 + 5 us
-// (5.0 TB/s); 16384 x 4096 bf16 107 us (5.0 TB/s) and 128 + 5 us (4.2 TB/s).  One row of 2048: 2.7 us.
+// Measured, with a residual: 786432 x 64 fp32 forward 135 us (6.0 TB/s, some of it from the last-level cache), backward 163 + 5 us
+// (5.0 TB/s); 16384 x 4096 bf16 109 us (4.9 TB/s) and 127 + 5 us (4.2 TB/s).  One row of 2048: 2.8 us.  Rows that the backward pass reads
+// twice, fp32 4096 x 8192: forward 112 us (4.8 TB/s), backward 207 us (2.6 TB/s).
 #include <type_traits>
 
 #include "layers_common.h"

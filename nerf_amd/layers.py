@@ -8,6 +8,9 @@ modules of nets.py do.  Element types: float32, float16, bfloat16.  Sums are hel
 same bits every time, gradients included.  Calls go to the device of their tensors and that device's current stream; workspaces
 come from torch's allocator on every call, so calls may overlap, and be captured into graphs, freely.
 
+Derivatives are those of torch.autograd's backward pass, once.  Forward-mode tangents, torch.func's transforms and make_fx are refused;
+torch.jit.trace records the calls.
+
 Capturing a backward pass: as with every torch autograd graph, no eager graph of the same leaves may be alive then (its
 gradient accumulation belongs to the stream it ran on); ``torch.autograd.grad`` inside the capture avoids accumulation altogether.
 """
@@ -108,7 +111,7 @@ def embedding(index, table, scale=1.0):
     """scale * table[index]: index int64 [...], table [n_entries, dim] -> [..., dim] of the table's type.
 
     An index outside [0, n_entries) gives a row of zeros and no gradient (nets.py:132 raises there; a kernel cannot).  The
-    table's gradient is dense and adds the rows of each entry in ascending order of their place in `index`."""
+    table's gradient is dense; the rows of an entry are added in an order that `index` fixes."""
     call = _EmbeddingFn.apply if _recorded(table, index) else _embedding_fwd
     return call(table, index, float(scale))
 
