@@ -31,14 +31,14 @@ ACTIVATIONS = {'silu': 0, 'gelu': 1, 'relu': 2}
 _current_device, _current_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 _transforms, _tracing = torch._C._functorch.peek_interpreter_stack, torch._C._get_tracing_state
 _modes, _mode_of = torch._C._len_torch_dispatch_stack, torch._C._get_dispatch_mode
-_includes, _early_mode_of = torch._C._dispatch_tls_is_dispatch_key_included, torch._ops._get_dispatch_mode_pre_dispatch
-_EARLY, _PROXY = torch._C.DispatchKey.PreDispatch, torch._C._TorchDispatchModeKey.PROXY
+_early_modes, _early_mode_of = torch._ops._len_torch_dispatch_stack_pre_dispatch, torch._ops._get_dispatch_mode_pre_dispatch
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
 
 
 def _launch(device, fn, what, *args):
     """fn(*args, stream): on the tensors' device, made current for the launch, and that device's current stream."""
     # make_fx on real tensors, also above autograd: it would record the allocation and not the launch
-    if _modes() and _mode_of(_PROXY) is not None or _includes(_EARLY) and _early_mode_of(_PROXY) is not None:
+    if _modes() and _mode_of(_PROXY) is not None or _early_modes() and _early_mode_of(_PROXY) is not None:
         raise RuntimeError('%s: a graph of torch operations cannot hold this kernel (torch.fx.experimental.proxy_tensor.make_fx)' % what)
     if device == _current_device():
         rc = fn(*args, _current_stream(device))

@@ -87,3 +87,22 @@ def test_calls_of_several_threads():
     assert not failed, failed
     for a, b in zip(alone, got):
         assert all(torch.equal(q, r) for q, r in zip(a, b))
+
+
+@pytest.mark.filterwarnings('ignore')
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+def test_a_compiled_trunk_is_the_trunk(backend):
+    net = Trunk()
+    index = torch.randint(0, 11, (300,), generator=torch.Generator().manual_seed(3)).cuda()
+    feats, dy = randn(300, 48, seed=8), randn(300, 3, seed=9)
+    params = list(net.parameters())
+    torch._dynamo.reset()
+    compiled = torch.compile(net, backend=backend)
+    for _ in range(2):
+        got, want = compiled(index, feats), net(index, feats)
+        assert torch.equal(got.detach(), want.detach())
+        for a, b in zip(torch.autograd.grad(got, params, dy), torch.autograd.grad(want, params, dy)):
+            assert torch.equal(a, b)
+    with torch.no_grad():
+        assert torch.equal(compiled(index, feats), net(index, feats))
+    torch._dynamo.reset()

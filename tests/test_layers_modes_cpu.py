@@ -142,3 +142,18 @@ def test_a_graph_of_operations_is_refused(standin, name, mode):
             make_fx(call, tracing_mode=mode, pre_dispatch=True)(x)
         with FlopCounterMode(display=False):
             assert close(call(x).detach(), plain(x))
+
+
+@pytest.mark.filterwarnings('ignore')
+@pytest.mark.parametrize('backend', ['eager', 'aot_eager'])
+@pytest.mark.parametrize('name', list(CALLS))
+def test_a_compiled_program_calls_out_of_its_graph(standin, name, backend):
+    """torch.compile breaks its graph at the launch and makes the call itself."""
+    call, plain = CALLS[name]
+    for leaf in (False, True):
+        torch._dynamo.reset()
+        compiled = torch.compile(lambda q: call(q * 2) + 1, backend=backend)
+        for rows in (4, 6):
+            x = randn(rows, 8, seed=rows).requires_grad_(leaf)
+            assert close(compiled(x).detach(), plain(x.detach() * 2) + 1)
+    torch._dynamo.reset()
