@@ -9,7 +9,7 @@ same bits every time, gradients included.  Calls go to the device of their tenso
 come from torch's allocator on every call, so calls may overlap, and be captured into graphs, freely.
 
 Derivatives are those of torch.autograd's backward pass, once.  Forward-mode tangents, torch.func's transforms and make_fx are refused;
-torch.jit.trace records the calls.
+torch.jit.trace records the calls, torch.compile breaks its graph at them.
 
 Capturing a backward pass: as with every torch autograd graph, no eager graph of the same leaves may be alive then (its
 gradient accumulation belongs to the stream it ran on); ``torch.autograd.grad`` inside the capture avoids accumulation altogether.
